@@ -14,7 +14,8 @@
 //
 // What bounds it: bytes (3 to 9 per element) at large T, launch latency at small T.  A block (or a
 // warp) keeps its row in registers between the passes over it (sum of squares, maximum, codes).
-// On a B200 (6.47 TB/s copies): 16384 x 2560 with y 49 us, 5.9 TB/s; 131072 x 2048 plain 116 us, 6.9 TB/s.
+// On a B200 (6.47 TB/s copies), back to back in a graph: 16384 x 2560 with y 50 us, 5.8 TB/s; 131072 x 2048 plain 115 us (134 us a
+// call in a loop, 6.0 TB/s: the shorter time leaves a tenth of the stores in L2).
 #include "kernels.h"
 #include "q4t_device.cuh"
 
@@ -35,6 +36,21 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return r;
 }
 
+// The codes of v / scale from ninv, minus the rounded 1 / scale: the product's error comes back as an exact remainder (Markstein's
+// correction of a quotient).  Checked against the division for all 2^23 mantissas of scale around the rounding borders of e4m3: of the
+// seven values of v next to a border the product alone puts 8 % on its wrong side, this none; bf16 rows lie on the borders often (four to
+// seven codes in ten thousand differed).  The quotients are formed negated, Q = v * ninv, Q - (v + Q scale) / scale, and the codes' signs
+// flipped back (flip: 0x80808080, or 0 in a row of NaNs): so an exact remainder, which is always +0, leaves the sign of a zero alone.
+__device__ __forceinline__ uint32_t quotients4(const float* v, uint64_t scale2, uint64_t ninv2, uint32_t flip) {
+  float q[4];
+#pragma unroll
+  for (int j = 0; j < 4; j += 2) {
+    const uint64_t v2 = f32x2(v[j], v[j + 1]), q2 = mul2(v2, ninv2);
+    f32x2_split(fma2(fma2(q2, scale2, v2), ninv2, q2), q[j], q[j + 1]);
+  }
+  return e4m3x4(q[0], q[1], q[2], q[3]) ^ flip;
+}
+
 // bf16(a + b) of a pair, added in fp32.
 __device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
   return f32x2_to_bf16x2(bf16x2_lo(a) + bf16x2_lo(b), bf16x2_hi(a) + bf16x2_hi(b));
@@ -42,7 +58,7 @@ __device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
 
 // WARPS: every warp of the block has a row of its own (no barriers); otherwise the block has one row.
 template <bool NORM, int G, bool WARPS>
-__global__ void __launch_bounds__(WARPS ? 256 : 1024) fp8_rows_kernel(const Fp8RowsArgs a, int rows) {
+__global__ void __launch_bounds__(WARPS ? 256 : 1024, WARPS || NORM ? 1 : 2) fp8_rows_kernel(const Fp8RowsArgs a, int rows) {
   __shared__ float s_sum[32];
   __shared__ uint32_t s_max[32];
   chain_wait();
@@ -108,17 +124,20 @@ __global__ void __launch_bounds__(WARPS ? 256 : 1024) fp8_rows_kernel(const Fp8R
     }
   }
 
-  float v[G][8];
+  float v[NORM ? G : 1][8];   // the plain quantiser unpacks its row where it needs it: registers are resident blocks
   uint32_t top = 0;
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
+  auto unpack = [&](int g, float (&f)[8]) {
     const uint32_t u[4] = {keep[g].x, keep[g].y, keep[g].z, keep[g].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      v[g][2 * j] = bf16x2_lo(u[j]);
-      v[g][2 * j + 1] = bf16x2_hi(u[j]);
+      f[2 * j] = bf16x2_lo(u[j]);
+      f[2 * j + 1] = bf16x2_hi(u[j]);
     }
-    if constexpr (NORM) {
+  };
+  if constexpr (NORM) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      unpack(g, v[g]);
       const uint32_t w[4] = {weight[g].x, weight[g].y, weight[g].z, weight[g].w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -129,11 +148,19 @@ __global__ void __launch_bounds__(WARPS ? 256 : 1024) fp8_rows_kernel(const Fp8R
           v[g][2 * j + 1] *= bf16x2_hi(w[j]) + a.weight_offset;
         }
       }
-    }
-    if (g * threads + tid < n8) {   // past the row 0 * rn may be a NaN
+      if (g * threads + tid < n8) {   // past the row 0 * rn may be a NaN
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[g][j]) & 0x7fffffffu);
+        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[g][j]) & 0x7fffffffu);
+      }
     }
+  } else {   // the bf16 patterns themselves, two at a time; past the row they are zeros
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const uint32_t u[4] = {keep[g].x, keep[g].y, keep[g].z, keep[g].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = __vmaxu2(top, u[j] & 0x7fff7fffu);
+    }
+    top = max(top & 0xffffu, top >> 16) << 16;
   }
   top = __reduce_max_sync(0xffffffffu, top);
   if (nw > 1) {
@@ -143,19 +170,22 @@ __global__ void __launch_bounds__(WARPS ? 256 : 1024) fp8_rows_kernel(const Fp8R
   }
   float scale = __fdiv_rn(fmaxf(__uint_as_float(top), kMinAmax), kE4m3Max);
   if (top >= 0x7f800000u) scale = __int_as_float(0x7fc00000);
-  const float inv = __frcp_rn(scale);
+  const uint32_t flip = top >= 0x7f800000u ? 0u : 0x80808080u;
+  const float ninv = -__frcp_rn(scale);
+  const uint64_t scale2 = f32x2(scale, scale), ninv2 = f32x2(ninv, ninv);
   if (tid == 0) a.scales[row] = scale;
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     const int i = g * threads + tid;
     if (i < n8) {
+      float(&f)[8] = v[NORM ? g : 0];
+      if constexpr (!NORM) unpack(g, f);
       reinterpret_cast<uint2*>(a.codes + row * a.hs)[i] =
-          make_uint2(e4m3x4(v[g][0] * inv, v[g][1] * inv, v[g][2] * inv, v[g][3] * inv),
-                     e4m3x4(v[g][4] * inv, v[g][5] * inv, v[g][6] * inv, v[g][7] * inv));
+          make_uint2(quotients4(&f[0], scale2, ninv2, flip), quotients4(&f[4], scale2, ninv2, flip));
       if (NORM && a.h)
         reinterpret_cast<uint4*>(a.h + row * a.hs)[i] =
-            make_uint4(f32x2_to_bf16x2(v[g][0], v[g][1]), f32x2_to_bf16x2(v[g][2], v[g][3]),
-                       f32x2_to_bf16x2(v[g][4], v[g][5]), f32x2_to_bf16x2(v[g][6], v[g][7]));
+            make_uint4(f32x2_to_bf16x2(f[0], f[1]), f32x2_to_bf16x2(f[2], f[3]), f32x2_to_bf16x2(f[4], f[5]),
+                       f32x2_to_bf16x2(f[6], f[7]));
     }
   }
 }
@@ -172,10 +202,10 @@ template <bool NORM>
 cudaError_t launch_rows(const Fp8RowsArgs& a, int rows, cudaStream_t stream) {
   // groups of eight elements a thread.  Few rows: one, the shortest chain of loads (one row of 2048: 1.8 us, four
   // groups 2.8).  Many rows: two, more bytes in flight without spending the registers that keep blocks resident (16384 x
-  // 2560: 49 us, one group 57, four 65).  Short rows with a warp each: 100000 blocks of one row of 72 took 53 us, this 15.
+  // 2560: 50 us, one group 57, four 65).  Short rows with a warp each: 100000 blocks of one row of 72 took 53 us, this 15.
   if (rows > 1024 && a.hs <= 256) return launch_groups<NORM, 1>(a, true, rows, stream);
   if (rows > 1024 && a.hs <= 512) return launch_groups<NORM, 2>(a, true, rows, stream);
-  if constexpr (!NORM)   // 20000 x 1016: 11.5 us, a block each 12.5; the norm's x, y and weights would be 86 registers: 24.1, 21.3
+  if constexpr (!NORM)   // 20000 x 1016: 10.8 us, a block each 12.5; the norm's x, y and weights would be 86 registers: 24.1, 21.3
     if (rows > 1024 && a.hs <= 1024) return launch_groups<NORM, 4>(a, true, rows, stream);
   if (rows <= 1024 && a.hs <= 8192) return launch_groups<NORM, 1>(a, false, rows, stream);
   if (a.hs <= 16384) return launch_groups<NORM, 2>(a, false, rows, stream);

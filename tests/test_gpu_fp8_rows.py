@@ -150,3 +150,46 @@ def test_on_another_stream_and_in_a_graph(q4t, gpu_lib):
     graph.replay()
     q4t.residual_rmsnorm_fp8(x, y, w, want, swant, x_out=torch.empty_like(x))
     assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8)) and torch.equal(scales, swant)
+
+
+def division(v):
+    """scale and e4m3(v / scale) of fp32 rows, with the divisions' own roundings (tensor by tensor: by a Python number a GPU tensor is
+    multiplied with the number's reciprocal)."""
+    top = v.abs().amax(dim=1).clamp_min(MIN_AMAX)
+    scale = top / torch.full_like(top, 448.0)
+    return (v / scale[:, None]).clamp(-448.0, 448.0).to(torch.float8_e4m3fn), scale
+
+
+def bf16_rows(rows, K, seed):
+    """Values of many magnitudes; few-bit ones among them, whose quotients lie on rounding borders."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(rows, K, generator=g, device="cuda") * torch.exp2(torch.randint(-60, 60, (rows, 1), generator=g, device="cuda").float())
+    few = torch.randint(0, 32, (rows, K), generator=g, device="cuda").float() * torch.exp2(torch.randint(-8, 4, (rows, K), generator=g, device="cuda").float())
+    x[::3] = (few * torch.where(torch.rand(rows, K, generator=g, device="cuda") < 0.5, -1.0, 1.0))[::3]
+    x[1] = 0.0
+    x[2, ::2] = -0.0
+    return x.bfloat16()
+
+
+@pytest.mark.parametrize("rows,K", [(96, 2560), (1201, 248), (1030, 504), (1100, 1016), (2050, 2048), (7, 8200), (3, 32768)])
+def test_codes_are_the_division(q4t, gpu_lib, rows, K):
+    """code = e4m3(v / scale) and scale = max / 448 bit for bit (v / scale rounded to fp32 first), signs of zeros included."""
+    x = bf16_rows(rows, K, rows + K)
+    codes, scales = q4t.quantize_rows_fp8(x)
+    want, swant = division(x.float())
+    assert torch.equal(scales, swant)
+    assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8))
+
+
+@pytest.mark.parametrize("T,hs", [(3, 2048), (1030, 248), (1100, 512), (1050, 2560), (5, 16384), (2, 32768)])
+def test_codes_of_a_norm_are_the_division(q4t, gpu_lib, T, hs):
+    """Rows of ones of either sign have an rms of exactly one: v is the weight."""
+    g = torch.Generator(device="cuda").manual_seed(T)
+    sign = torch.where(torch.rand(T, hs, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    for i in range(3):
+        w = bf16_rows(3, hs, hs + i)[i if i != 1 else 2]
+        codes, scales = outputs(T, hs)
+        q4t.residual_rmsnorm_fp8(sign.bfloat16(), None, w, codes, scales, eps=0.0)
+        want, swant = division(sign * (w.float() + 0.0))   # the offset of zero takes the weight's -0 away
+        assert torch.equal(scales, swant)
+        assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8))
