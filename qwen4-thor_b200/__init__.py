@@ -683,12 +683,25 @@ class DecodeStack:
                                           float(self.eps), sp))
         return x
 
+    def _check_x(self, x):
+        """The stack takes x as an address: the rows that it adds to have to be there."""
+        import torch
+        shape = (self.T, self.layers[0].hs)
+        if not isinstance(x, torch.Tensor) or x.dtype != torch.bfloat16 or x.shape != shape or not x.is_contiguous():
+            what = f"{x.dtype} {tuple(x.shape)}" if isinstance(x, torch.Tensor) else type(x).__name__
+            raise Q4TError(f"x: contiguous torch.bfloat16 {shape} is needed, not {what}")
+        if not x.is_cuda or x.device != self.h.device:
+            raise Q4TError(f"x: a CUDA tensor on the stack's device {self.h.device} is needed, not one on {x.device}")
+        if x.data_ptr() % 16:
+            raise Q4TError("x: rows must be 16-byte aligned")
+
     def verify(self, x, head: "VerifyHead", draft_ids, uniforms, draft_logits=None, temperature=None, draft_len=None,
                stream=None):
         """One decode step with speculative verification: the stack in place on x (one row per target and draft
         position), then the verify head on what it leaves.  Arguments and result as in VerifyHead."""
         if head.T != self.T:
             raise Q4TError(f"verify: the head takes {head.T} rows, the stack {self.T}")
+        self._check_x(x)
         head.verifier.check(draft_ids, uniforms, draft_logits, temperature, draft_len)
         self(x, stream)
         return head(x, draft_ids, uniforms, draft_logits=draft_logits, temperature=temperature, draft_len=draft_len,

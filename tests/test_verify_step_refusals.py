@@ -207,3 +207,33 @@ def test_verify_head_shape(q4t):
     for shape, fp8 in (((32, 24), True), ((32, 12), False), ((32,), True)):
         with pytest.raises(q4t.Q4TError, match="head_weight"):
             q4t.VerifyHead(None, torch.zeros(shape, dtype=torch.bfloat16), 1, 1, fp8=fp8)
+
+
+@pytest.fixture
+def step(q4t, monkeypatch):
+    """A stack and a head that fits it, on the host; the list grows when the stack runs."""
+    ran = []
+    monkeypatch.setattr(q4t.DecodeStack, "__call__", lambda self, x, stream=None: ran.append(x))
+    stack = object.__new__(q4t.DecodeStack)
+    stack.layers, stack.T, stack.h = [type("Layer", (), {"hs": 256})()], 6, torch.empty(6, 256, dtype=torch.bfloat16)
+    return stack, q4t.VerifyHead(None, torch.zeros(100, 256, dtype=torch.bfloat16), 2, 2, fp8=False), ran
+
+
+IDS, U = torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, 3)
+
+
+@pytest.mark.parametrize("x,text", [(torch.zeros(5, 256, dtype=torch.bfloat16), "contiguous"),           # too few rows
+                                    (torch.zeros(7, 256, dtype=torch.bfloat16), "contiguous"),
+                                    (torch.zeros(6, 128, dtype=torch.bfloat16), "contiguous"),
+                                    (torch.zeros(6 * 256, dtype=torch.bfloat16), "contiguous"),
+                                    (torch.zeros(6, 512, dtype=torch.bfloat16)[:, ::2], "contiguous"),   # strided
+                                    (torch.zeros(6, 320, dtype=torch.bfloat16)[:, :256], "contiguous"),
+                                    (torch.zeros(6, 256), "contiguous"),                                # another type
+                                    (torch.zeros(6, 256, dtype=torch.float16), "contiguous"),
+                                    (None, "contiguous"),
+                                    (torch.zeros(6, 256, dtype=torch.bfloat16), "CUDA tensor")])
+def test_rows_that_the_stack_would_read_past_are_refused(q4t, step, x, text):
+    stack, head, ran = step
+    with pytest.raises(q4t.Q4TError, match=text):
+        stack.verify(x, head, IDS, U)
+    assert not ran
