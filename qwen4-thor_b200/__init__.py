@@ -701,6 +701,9 @@ class DecodeStack:
         position), then the verify head on what it leaves.  Arguments and result as in VerifyHead."""
         if head.T != self.T:
             raise Q4TError(f"verify: the head takes {head.T} rows, the stack {self.T}")
+        if head.codes.shape[1] != self.layers[0].hs or head.codes.device != self.h.device:
+            raise Q4TError(f"verify: the head takes rows of {head.codes.shape[1]} on {head.codes.device}, the stack has {self.layers[0].hs} "
+                           f"on {self.h.device}")
         self._check_x(x)
         head.verifier.check(draft_ids, uniforms, draft_logits, temperature, draft_len)
         self(x, stream)

@@ -219,3 +219,15 @@ def test_refused_steps_change_nothing(q4t, gpu_lib):
         with pytest.raises(q4t.Q4TError):
             head(x, y=x.clone(), **args)
     assert torch.equal(x, before)
+
+
+def test_a_head_that_does_not_fit_is_refused_before_x_changes(q4t, gpu_lib):
+    dl = q4t.DeviceLayer.from_host(synth.make_layer(E=8, hs=256, moe_is=128, shared_is=128, seed=1))
+    stack = q4t.DecodeStack([dl], 6, 2)
+    x = torch.randn(6, 256, device="cuda").bfloat16()
+    before = x.clone()
+    ids, u = torch.zeros(2, 2, dtype=torch.int32, device="cuda"), torch.zeros(2, 3, device="cuda")
+    nw, w = head_weights(100, 512, 5)
+    with pytest.raises(q4t.Q4TError):
+        stack.verify(x, q4t.VerifyHead(nw, w, 2, 2), ids, u)
+    assert torch.equal(x, before)

@@ -237,3 +237,11 @@ def test_rows_that_the_stack_would_read_past_are_refused(q4t, step, x, text):
     with pytest.raises(q4t.Q4TError, match=text):
         stack.verify(x, head, IDS, U)
     assert not ran
+
+
+def test_a_head_of_other_rows_is_refused_before_the_stack_runs(q4t, step):
+    stack, head, ran = step
+    other = q4t.VerifyHead(None, torch.zeros(100, 512, dtype=torch.bfloat16), 2, 2, fp8=False)
+    with pytest.raises(q4t.Q4TError, match="the head takes rows of 512"):
+        stack.verify(torch.zeros(6, 256, dtype=torch.bfloat16), other, IDS, U)
+    assert not ran
