@@ -725,6 +725,19 @@ class VerifyHead:
             raise Q4TError(f"head_weight: [V, hs] with hs a multiple of {16 if fp8 else 8} is needed, not {tuple(head_weight.shape)}")
         V, hs = head_weight.shape
         T, device = B * (n + 1), head_weight.device
+        # all that a step would refuse of these, here: x may have changed by then
+        if head_weight.dtype != torch.bfloat16 or hs > 32768:
+            raise Q4TError(f"head_weight: torch.bfloat16 with hs at most 32768 is needed, not {head_weight.dtype} {tuple(head_weight.shape)}")
+        if not fp8 and ((hs > 1 and head_weight.stride(1) != 1) or head_weight.data_ptr() % 16 or
+                        (V > 1 and (head_weight.stride(0) < hs or head_weight.stride(0) % 8))):
+            raise Q4TError("head_weight: contiguous rows that start on 16 bytes are needed")
+        if norm_weight is not None and (not isinstance(norm_weight, torch.Tensor) or norm_weight.dtype != torch.bfloat16 or
+                                        norm_weight.shape != (hs,) or norm_weight.device != device or
+                                        not norm_weight.is_contiguous() or norm_weight.data_ptr() % 16):
+            raise Q4TError(f"norm_weight: contiguous torch.bfloat16 ({hs},) on {device}, 16-byte aligned, or None is needed")
+        if not float(eps) >= 0.0:
+            raise Q4TError(f"eps: {eps} is negative or not a number")
+        weight_offset = float(weight_offset)
         self.norm_weight, self.eps, self.weight_offset, self.fp8, self.T = norm_weight, eps, weight_offset, fp8, T
         self.head, self.head_scale = quantize_rows_fp8(head_weight) if fp8 else (head_weight, None)
         self.codes = torch.empty((T, hs), dtype=torch.float8_e4m3fn, device=device)

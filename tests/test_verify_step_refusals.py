@@ -245,3 +245,23 @@ def test_a_head_of_other_rows_is_refused_before_the_stack_runs(q4t, step):
     with pytest.raises(q4t.Q4TError, match="the head takes rows of 512"):
         stack.verify(torch.zeros(6, 256, dtype=torch.bfloat16), other, IDS, U)
     assert not ran
+
+
+def test_weights_that_no_step_could_use_are_refused_with_the_head(q4t):
+    def head(norm=None, w=torch.zeros(100, 256, dtype=torch.bfloat16), eps=1e-6, fp8=False):
+        return q4t.VerifyHead(norm, w, 2, 2, eps=eps, fp8=fp8)
+    good = torch.zeros(256, dtype=torch.bfloat16)
+    assert head(good).T == 6 and head().T == 6
+    assert head(w=torch.zeros(100, 272, dtype=torch.bfloat16)[:, :256]).T == 6      # rows further apart
+    for bad in (good.float(), good[:128], torch.zeros(512, dtype=torch.bfloat16)[::2], good.view(1, 256), 1.0,
+                torch.zeros(264, dtype=torch.bfloat16)[4:260]):
+        with pytest.raises(q4t.Q4TError, match="norm_weight"):
+            head(bad)
+    wide = torch.zeros(100, 264, dtype=torch.bfloat16)
+    for bad in (torch.zeros(100, 256), torch.zeros(2, 32776, dtype=torch.bfloat16), torch.zeros(256, 100, dtype=torch.bfloat16).t(),
+                wide[:, 4:260], torch.zeros(100, 260, dtype=torch.bfloat16)[:, :256], good.expand(100, 256)):
+        with pytest.raises(q4t.Q4TError, match="head_weight"):
+            head(w=bad)
+    for eps in (-1e-6, float("nan")):
+        with pytest.raises(q4t.Q4TError, match="eps"):
+            head(eps=eps)
