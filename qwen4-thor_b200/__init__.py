@@ -625,6 +625,10 @@ class VerifyDrafts:
             dense = t.stride(1) == 1 or V == 1 if name == "draft_logits" else t.is_contiguous()
             if t.dtype != dtype or t.device != self.ws.device or not dense:
                 raise Q4TError(f"{name}: contiguous {dtype} on {self.ws.device} is needed, not {t.dtype} on {t.device}")
+            if name == "draft_logits" and B * n > 1 and t.stride(0) < V:
+                raise Q4TError(f"{name}: rows overlap (stride {t.stride(0)})")
+            if t.data_ptr() % t.element_size():
+                raise Q4TError(f"{name}: must be aligned to its type")
 
     def __call__(self, target_logits, draft_ids, uniforms, tokens=None, accepted=None, probs=None, draft_logits=None,
                  temperature=None, draft_len=None, stream=None):

@@ -231,3 +231,19 @@ def test_a_head_that_does_not_fit_is_refused_before_x_changes(q4t, gpu_lib):
     with pytest.raises(q4t.Q4TError):
         stack.verify(x, q4t.VerifyHead(nw, w, 2, 2), ids, u)
     assert torch.equal(x, before)
+
+
+def test_overlapping_draft_rows_are_refused_before_x_changes(q4t, gpu_lib):
+    dl = q4t.DeviceLayer.from_host(synth.make_layer(E=8, hs=256, moe_is=128, shared_is=128, seed=1))
+    nw, w = head_weights(100, 256, 5)
+    stack, head = q4t.DecodeStack([dl], 6, 2), q4t.VerifyHead(nw, w, 2, 2)
+    x = torch.randn(6, 256, device="cuda").bfloat16()
+    before = x.clone()
+    ids, u = torch.zeros(2, 2, dtype=torch.int32, device="cuda"), torch.zeros(2, 3, device="cuda")
+    one = torch.zeros(1, 100, device="cuda").bfloat16()
+    for bad in (one.expand(4, 100), torch.zeros(200, device="cuda").bfloat16().as_strided((4, 100), (30, 1))):
+        with pytest.raises(q4t.Q4TError):
+            stack.verify(x, head, ids, u, draft_logits=bad)
+        with pytest.raises(q4t.Q4TError):
+            head(x, ids, u, y=x.clone(), draft_logits=bad)
+    assert torch.equal(x, before)

@@ -265,3 +265,16 @@ def test_weights_that_no_step_could_use_are_refused_with_the_head(q4t):
     for eps in (-1e-6, float("nan")):
         with pytest.raises(q4t.Q4TError, match="eps"):
             head(eps=eps)
+
+
+def test_draft_rows_that_overlap_are_refused_by_the_check(q4t):
+    v = q4t.VerifyDrafts(2, 2, 100, device="cpu")
+    bf16 = torch.bfloat16
+    v.check(IDS, U)
+    for good in (torch.zeros(4, 100, dtype=bf16), torch.zeros(4, 107, dtype=bf16)[:, :100], torch.zeros(4, 101, dtype=bf16)[:, 1:]):
+        v.check(IDS, U, good)
+    for bad in (torch.zeros(1, 100, dtype=bf16).expand(4, 100), torch.zeros(400, dtype=bf16).as_strided((4, 100), (99, 1))):
+        with pytest.raises(q4t.Q4TError, match="rows overlap"):
+            v.check(IDS, U, bad)
+    one = q4t.VerifyDrafts(1, 1, 100, device="cpu")      # the stride of a single row does not matter
+    one.check(IDS[:1, :1], U[:1, :2], torch.zeros(100, dtype=bf16).as_strided((1, 100), (0, 1)))
