@@ -708,6 +708,7 @@ class DecodeStack:
         if head.codes.shape[1] != self.layers[0].hs or head.codes.device != self.h.device:
             raise Q4TError(f"verify: the head takes rows of {head.codes.shape[1]} on {head.codes.device}, the stack has {self.layers[0].hs} "
                            f"on {self.h.device}")
+        head._check_drafts(draft_logits)
         self._check_x(x)
         head.verifier.check(draft_ids, uniforms, draft_logits, temperature, draft_len)
         self(x, stream)
@@ -750,9 +751,16 @@ class VerifyHead:
         self.logits = torch.empty((T, V), dtype=torch.bfloat16, device=device)
         self.verifier = VerifyDrafts(B, n, V, device=device)   # behind the weight's layout: waits for that too
 
+    def _check_drafts(self, draft_logits):
+        """The product writes self.logits before the drafts' logits are read."""
+        if draft_logits is not None and hasattr(draft_logits, "untyped_storage"):
+            if draft_logits.untyped_storage().data_ptr() == self.logits.untyped_storage().data_ptr():
+                raise Q4TError("draft_logits: lie in the head's own logits, which the step overwrites (pass a copy)")
+
     def __call__(self, x, draft_ids, uniforms, y=None, draft_logits=None, temperature=None, draft_len=None, stream=None):
         """x: residual stream bf16 [T, hs] (y, if given, is added to it first, in place); the rest as in VerifyDrafts.
         Returns {tokens, accepted, probs}; the logits stay in self.logits."""
+        self._check_drafts(draft_logits)
         if y is not None:   # x is about to change
             self.verifier.check(draft_ids, uniforms, draft_logits, temperature, draft_len)
         residual_rmsnorm_fp8(x, y, self.norm_weight, self.codes, self.scales, x_out=None if y is None else x, h=self.h,

@@ -278,3 +278,14 @@ def test_draft_rows_that_overlap_are_refused_by_the_check(q4t):
             v.check(IDS, U, bad)
     one = q4t.VerifyDrafts(1, 1, 100, device="cpu")      # the stride of a single row does not matter
     one.check(IDS[:1, :1], U[:1, :2], torch.zeros(100, dtype=bf16).as_strided((1, 100), (0, 1)))
+
+
+def test_draft_logits_in_the_logits_of_the_step_are_refused(q4t, step):
+    """They would be overwritten before they are read."""
+    stack, head, ran = step
+    for bad in (head.logits[:4], head.logits[2:]):
+        with pytest.raises(q4t.Q4TError, match="head's own logits"):
+            stack.verify(torch.zeros(6, 256, dtype=torch.bfloat16), head, IDS, U, draft_logits=bad)
+        with pytest.raises(q4t.Q4TError, match="head's own logits"):
+            head(torch.zeros(6, 256, dtype=torch.bfloat16), IDS, U, draft_logits=bad)
+    assert not ran
