@@ -580,7 +580,8 @@ int32_t q4t_quantize_rows_fp8(const uint16_t* x, uint8_t* codes, float* scales,
 
 /* A linear layer with everything behind the product in its epilogue:
  *   out[m, n] = round(act(acc * x_scale[m] * w_scale[n] + bias[n]) + residual[m, n]),
- *   acc = sum_k x[m, k] * w[n, k] in fp32, one rounding to the type of out.
+ *   acc = sum_k x[m, k] * w[n, k] in fp32, the scales applied in this order (their product may
+ *   leave fp32 where the result does not), one rounding to the type of out.
  * Operands both bf16, or (fp8 != 0) both e4m3 with an fp32 scale per row (as
  * q4t_residual_rmsnorm_fp8 and q4t_quantize_rows_fp8 leave them; NULL: 1).  act: none,
  * SiLU v / (1 + e^-v), or GELU in its tanh form.  Any M, N, K; rows of x and w start on

@@ -100,7 +100,7 @@ __device__ __forceinline__ void finish4(const LinearArgs& a, int m, int n, int n
                                         const float (&ws)[4], const float (&bias)[4], uint2 res) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (FP8) o[i] *= xs * ws[i];
+    if (FP8) o[i] = o[i] * xs * ws[i];   // in turn: the scales' product may leave fp32 where the result does not
     o[i] = activate<ACT>(o[i] + bias[i]);
   }
   o[0] += bf16x2_lo(res.x);
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(256) linear_row_kernel(const __grid_constant__
   // what the epilogue reads is requested with the operands: lane i of the first share finishes output n0 + i
   const int n = n0 + lane;
   const bool finishes = lane < R && share == 0 && n < a.N;
-  const float ws = FP8 && finishes ? (a.x_scale ? a.x_scale[0] : 1.0f) * (a.w_scale ? a.w_scale[n] : 1.0f) : 1.0f;
+  const float xs = FP8 && finishes && a.x_scale ? a.x_scale[0] : 1.0f, ws = FP8 && finishes && a.w_scale ? a.w_scale[n] : 1.0f;
   const float bias = finishes && a.bias ? bf16_to_f32(a.bias[n]) : 0.0f;
   const float residual = finishes && a.residual ? bf16_to_f32(a.residual[n]) : 0.0f;
   float acc[R];
@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(256) linear_row_kernel(const __grid_constant__
 #pragma unroll
     for (int i = 1; i < R; ++i)
       if (lane == i) v = acc[i];
-    if (FP8) v *= ws;
+    if (FP8) v = v * xs * ws;   // in turn, see finish4
     v += bias;
     v = a.act == kLinSilu ? activate<kLinSilu>(v) : a.act == kLinGelu ? activate<kLinGelu>(v) : v;
     v += residual;
