@@ -584,7 +584,9 @@ int32_t q4t_quantize_rows_fp8(const uint16_t* x, uint8_t* codes, float* scales,
  *   leave fp32 where the result does not), one rounding to the type of out.
  * Operands both bf16, or (fp8 != 0) both e4m3 with an fp32 scale per row (as
  * q4t_residual_rmsnorm_fp8 and q4t_quantize_rows_fp8 leave them; NULL: 1).  act: none,
- * SiLU v / (1 + e^-v), or GELU in its tanh form.  Any M, N, K; rows of x and w start on
+ * SiLU v / (1 + e^-v), or GELU in its tanh form (both by the fast exponential and reciprocal,
+ * for fp32 outputs too: within (7 + 4 |s|) 2^-23 of the result, s the sigmoid's argument; results below
+ * 2^-126 may be zeros).  Any M, N, K; rows of x and w start on
  * 16 bytes (base and stride), rows of out and residual anywhere their type may.  out may
  * be residual (same type and stride); it may not overlap anything else (refused; columns of
  * one buffer may be out and an operand when both have its row stride).  M <= 0 is a

@@ -72,14 +72,16 @@ __device__ __forceinline__ void arrive_relaxed_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
-// v * sigmoid(s), s = v (SiLU) or 2 sqrt(2/pi) (v + 0.044715 v^3) (GELU, 0.5 v (1 + tanh(s/2))).  The exponential and the
-// division are the fast forms (a few ulp): two special-function operations an element instead of a division routine,
-// which cost more than the e4m3 mainloop of a K = 2560 tile.
+// v * sigmoid(s), s = v (SiLU) or 2 sqrt(2/pi) (v + 0.044715 v^3) (GELU, 0.5 v (1 + tanh(s/2))), from exp(-|s|), times 2^7 while it is a
+// number of its own: neither it nor the denominator, 1 .. 2, leaves fp32 before the result does.  (v / (1 + exp(-s)) by the fast division
+// is 0 where 1 + exp(-s) is above 2^126: SiLU of -88, 5e-37.)  Two special-function operations an element, good to 2^-22, instead of a
+// division routine, which cost more than the e4m3 mainloop of a K = 2560 tile.
 template <int ACT>
 __device__ __forceinline__ float activate(float v) {
-  if (ACT == kLinSilu) return __fdividef(v, 1.0f + __expf(-v));
-  if (ACT == kLinGelu) return __fdividef(v, 1.0f + __expf(-1.5957691216057308f * fmaf(0.044715f * v * v, v, v)));
-  return v;
+  if (ACT != kLinSilu && ACT != kLinGelu) return v;
+  const float u = ACT == kLinSilu ? v : fmaf(0.044715f * v * v, v, v);
+  const float e = ex2(fmaf(-fabsf(u), ACT == kLinSilu ? 1.4426950408889634f : 2.302208198144325f, 7.0f));   // log2(e), 2 sqrt(2/pi) log2(e)
+  return (v >= 0.0f ? v : v * e * 0.0078125f) * rcp(fmaf(e, 0.0078125f, 1.0f));
 }
 
 // The row's four values at a.residual + ..[m, n .. n + 3] as bf16 pairs; those past N read as zeros.

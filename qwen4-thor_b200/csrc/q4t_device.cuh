@@ -27,6 +27,18 @@ __device__ __forceinline__ uint32_t f32x2_to_bf16x2(float lo, float hi) {
 __device__ __forceinline__ float bf16x2_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf16x2_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
+// 2^z and 1 / d on the special-function unit; results below 2^-126 are zeros.
+__device__ __forceinline__ float ex2(float z) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(z));
+  return r;
+}
+__device__ __forceinline__ float rcp(float d) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return r;
+}
+
 // Two fp32 in one register pair: one instruction for two fused steps or sums.
 __device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
   uint64_t r;

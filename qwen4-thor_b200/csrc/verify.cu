@@ -133,12 +133,6 @@ struct Row {
   }
 };
 
-__device__ __forceinline__ float ex2(float z) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(z));
-  return r;
-}
-
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
