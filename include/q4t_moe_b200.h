@@ -610,6 +610,9 @@ typedef struct q4t_linear_args {
   void* out;                 /* [M, N] */
 } q4t_linear_args;
 int32_t q4t_linear(const q4t_linear_args* args, void* stream);
+/* What q4t_linear refuses of these arguments, on the host alone (no GPU needed): for callers that
+ * change something before they get to it.                                          */
+int32_t q4t_linear_check(const q4t_linear_args* args);
 /* Did a bounded device-side wait of q4t_linear run out on the current device since the
  * last call of this function?  Synchronise the stream first; Q4T_ERR_KERNEL if so
  * (the output was then not completed), 0 otherwise.                             */
@@ -653,6 +656,8 @@ typedef struct q4t_verify_args {
 size_t q4t_verify_drafts_workspace_bytes(int32_t B, int32_t n, int32_t V);
 int32_t q4t_verify_drafts(const q4t_verify_args* args, void* workspace, size_t workspace_bytes,
                           void* stream);
+/* What q4t_verify_drafts refuses of these arguments, on the host alone.           */
+int32_t q4t_verify_drafts_check(const q4t_verify_args* args, const void* workspace, size_t workspace_bytes);
 
 /* Reads the kernel status words of a workspace after the stream has been
  * synchronised by the caller: 0 = clean, otherwise a bounded device-side wait

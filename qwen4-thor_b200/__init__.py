@@ -100,7 +100,7 @@ EXPORTS = [
     "q4t_moe_bf16_forward",
     "q4t_peer_buffer_alloc", "q4t_peer_buffer_free", "q4t_peer_buffer_export", "q4t_peer_buffer_open",
     "q4t_peer_buffer_close", "q4t_ep_publish", "q4t_ep_publish_selected", "q4t_ep_route_publish", "q4t_ep_combine", "q4t_moe_expert_peer_workspace_bytes", "q4t_moe_expert_peer", "q4t_ep_flat_rows",
-    "q4t_residual_rmsnorm_fp8", "q4t_quantize_rows_fp8", "q4t_linear", "q4t_linear_status", "q4t_verify_drafts_workspace_bytes", "q4t_verify_drafts",
+    "q4t_residual_rmsnorm_fp8", "q4t_quantize_rows_fp8", "q4t_linear", "q4t_linear_check", "q4t_linear_status", "q4t_verify_drafts_workspace_bytes", "q4t_verify_drafts", "q4t_verify_drafts_check",
     "q4t_ep_sync_buffer_bytes", "q4t_ep_post_ids", "q4t_ep_post_rows", "q4t_ep_wait", "q4t_ep_sync_status",
 ]
 # libq4t_moe_b200_check.so (include/q4t_moe_b200_check.h): device-side checkers for the GPU tests only.
@@ -176,9 +176,11 @@ def load():
     L.q4t_residual_rmsnorm_fp8.argtypes = [vp, vp, vp, vp, f32, vp, vp, vp, i32, i32, f32, vp]
     L.q4t_quantize_rows_fp8.argtypes = [vp, vp, vp, i32, i32, vp]
     L.q4t_linear.argtypes = [C.POINTER(LinearArgs), vp]
+    L.q4t_linear_check.argtypes = [C.POINTER(LinearArgs)]
     L.q4t_verify_drafts_workspace_bytes.restype = sz
     L.q4t_verify_drafts_workspace_bytes.argtypes = [i32, i32, i32]
     L.q4t_verify_drafts.argtypes = [C.POINTER(VerifyArgs), vp, sz, vp]
+    L.q4t_verify_drafts_check.argtypes = [C.POINTER(VerifyArgs), vp, sz]
     L.q4t_ep_route_publish.argtypes = [vp, C.POINTER(ExtraWeights), C.POINTER(EpPeerTable), i32, f32, vp, vp, vp, vp,
                                        sz, vp]
     L.q4t_ep_combine.argtypes = [vp, vp, vp, vp, C.POINTER(ExtraWeights), vp, i32, i32, vp, vp, sz, vp]

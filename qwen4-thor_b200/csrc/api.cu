@@ -112,6 +112,83 @@ int fail_overlap(const char* out, const char* other) {
   return fail(Q4T_ERR_INVALID, std::string(out) + " overlaps " + other);
 }
 
+// The argument checks of q4t_linear for M > 0; the strides that its rows have.
+struct LinearStrides {
+  int64_t ldx, ldw, ldo, ldr;
+};
+int check_linear(const q4t_linear_args* l, LinearStrides* s) {
+  if (l->N <= 0 || l->K <= 0) return fail(Q4T_ERR_INVALID, "invalid GEMM dims");
+  if (!l->x || !l->w || !l->out) return fail(Q4T_ERR_INVALID, "null pointer");
+  if (l->activation < 0 || l->activation > Q4T_ACT_GELU) return fail(Q4T_ERR_INVALID, "unknown activation");
+  if (!l->fp8 && (l->x_scale || l->w_scale)) return fail(Q4T_ERR_INVALID, "scales belong to e4m3 operands");
+  const int64_t esz = l->fp8 ? 1 : 2;
+  // the stride of a single row is never used: any length of it will do
+  const int64_t one = (static_cast<int64_t>(l->K) + 15) & ~int64_t{15};
+  const int64_t ldx = s->ldx = l->M == 1 ? one : (l->ldx ? l->ldx : l->K), ldw = s->ldw = l->N == 1 ? one : (l->ldw ? l->ldw : l->K);
+  const int64_t ldo = s->ldo = l->ldo ? l->ldo : l->N, ldr = s->ldr = l->M == 1 ? ldo : (l->ldr ? l->ldr : l->N);
+  if (ldx < l->K || ldw < l->K || ldo < l->N || ldr < l->N) return fail(Q4T_ERR_INVALID, "a row stride is shorter than its row");
+  if (((reinterpret_cast<uintptr_t>(l->x) | reinterpret_cast<uintptr_t>(l->w)) & 15u) || (ldx * esz) % 16 || (ldw * esz) % 16)
+    return fail(Q4T_ERR_INVALID, "x and w must start at, and their rows be a multiple of, 16 bytes");
+  if (reinterpret_cast<uintptr_t>(l->out) % (l->out_f32 ? 4 : 2) || reinterpret_cast<uintptr_t>(l->residual) % 2 ||
+      reinterpret_cast<uintptr_t>(l->bias) % 2 || (reinterpret_cast<uintptr_t>(l->x_scale) | reinterpret_cast<uintptr_t>(l->w_scale)) % 4)
+    return fail(Q4T_ERR_INVALID, "out, residual, bias and scales must be aligned to their types");
+  if (l->residual && static_cast<const void*>(l->residual) == l->out && (l->out_f32 || ldr != ldo))
+    return fail(Q4T_ERR_INVALID, "in place, out and residual need the same type and row stride");
+  if (too_far(l->M, ldx, esz) || too_far(l->N, ldw, esz) || too_far(l->M, ldo, 4) || too_far(l->M, ldr, 2) || l->M > (1 << 30) || l->N > (1 << 30) || l->K > (1 << 29) || static_cast<int64_t>(l->N / 128 + 1) * (l->M / 16 + 1) > (1 << 30))
+    return fail(Q4T_ERR_INVALID, "dims too large");
+  // every output is finished by the thread that read its residual element: only there may the two be one
+  const bool in_place = static_cast<const void*>(l->residual) == l->out;
+  if (const char* on = covered(span_of(l->out, l->M, l->N, ldo, l->out_f32 ? 4 : 2),
+                               {{"x", span_of(l->x, l->M, l->K, ldx, esz)},
+                                {"w", span_of(l->w, l->N, l->K, ldw, esz)},
+                                {"x_scale", span_of(l->x_scale, int64_t{4} * l->M)},
+                                {"w_scale", span_of(l->w_scale, int64_t{4} * l->N)},
+                                {"bias", span_of(l->bias, int64_t{2} * l->N)},
+                                {"residual", span_of(in_place ? nullptr : l->residual, l->M, l->N, ldr, 2)}}))
+    return fail_overlap("out", on);
+  return Q4T_OK;
+}
+
+// The argument checks of q4t_verify_drafts for B > 0.
+int check_verify(const q4t_verify_args* v, const void* workspace, size_t workspace_bytes) {
+  if (v->n <= 0 || v->n > q4t::kVerifyMaxDrafts) return fail(Q4T_ERR_INVALID, "n out of range (1..64)");
+  if (v->V <= 0 || v->V > (1 << 30)) return fail(Q4T_ERR_INVALID, "V out of range (1..2^30)");
+  if (static_cast<int64_t>(v->B) * (2 * v->n + 1) > q4t::kVerifyMaxRows)
+    return fail(Q4T_ERR_INVALID, "too many rows: B * (2n + 1) is at most 65535");
+  if (!v->target_logits || !v->draft_ids || !v->uniforms || !v->tokens || !v->accepted)
+    return fail(Q4T_ERR_INVALID, "null pointer");
+  const int64_t tld = v->target_ld ? v->target_ld : v->V, dld = v->draft_ld ? v->draft_ld : v->V;
+  if (tld < v->V || dld < v->V) return fail(Q4T_ERR_INVALID, "a row stride is shorter than V");
+  if (too_far(q4t::kVerifyMaxRows, tld, 4) || too_far(q4t::kVerifyMaxRows, dld, 4)) return fail(Q4T_ERR_INVALID, "dims too large");
+  const uintptr_t esz = v->logits_f32 ? 4 : 2;
+  if ((reinterpret_cast<uintptr_t>(v->target_logits) | reinterpret_cast<uintptr_t>(v->draft_logits)) % esz)
+    return fail(Q4T_ERR_INVALID, "logits must be aligned to their type");
+  if ((reinterpret_cast<uintptr_t>(v->draft_ids) | reinterpret_cast<uintptr_t>(v->draft_len) | reinterpret_cast<uintptr_t>(v->temperature) |
+       reinterpret_cast<uintptr_t>(v->uniforms) | reinterpret_cast<uintptr_t>(v->tokens) | reinterpret_cast<uintptr_t>(v->accepted) |
+       reinterpret_cast<uintptr_t>(v->probs)) & 3u)
+    return fail(Q4T_ERR_INVALID, "ids, lengths, temperatures, uniforms and outputs must be 4-byte aligned");
+  const size_t need = q4t_verify_drafts_workspace_bytes(v->B, v->n, v->V);
+  if (!workspace || workspace_bytes < need) return fail(Q4T_ERR_WORKSPACE, "workspace too small");
+  if (reinterpret_cast<uintptr_t>(workspace) & 15u) return fail(Q4T_ERR_INVALID, "workspace must be 16-byte aligned");
+  const int64_t B = v->B, n = v->n;
+  const std::pair<const char*, Span> written[4] = {{"tokens", span_of(v->tokens, B * (n + 1) * 4)},
+                                                   {"accepted", span_of(v->accepted, B * 4)},
+                                                   {"probs", span_of(v->probs, B * (n + 1) * 4)},
+                                                   {"workspace", span_of(workspace, static_cast<int64_t>(need))}};
+  const std::pair<const char*, Span> read[6] = {{"target_logits", span_of(v->target_logits, B * (n + 1), v->V, tld, static_cast<int64_t>(esz))},
+                                                {"draft_logits", span_of(v->draft_logits, B * n, v->V, dld, static_cast<int64_t>(esz))},
+                                                {"draft_ids", span_of(v->draft_ids, B * n * 4)},
+                                                {"draft_len", span_of(v->draft_len, B * 4)},
+                                                {"temperature", span_of(v->temperature, B * 4)},
+                                                {"uniforms", span_of(v->uniforms, B * (n + 1) * 4)}};
+  for (int i = 0; i < 4; ++i) {
+    if (const char* on = covered(written[i].second, read)) return fail_overlap(written[i].first, on);
+    for (int j = 0; j < i; ++j)
+      if (overlap(written[i].second, written[j].second)) return fail_overlap(written[i].first, written[j].first);
+  }
+  return Q4T_OK;
+}
+
 // Per-device one-time set-up: architecture check, driver entry point for the
 // tensor-map encoder, shared-memory attribute of the GEMM kernels.
 int device_state(const DeviceState** out) {
@@ -1799,41 +1876,21 @@ int32_t q4t_quantize_rows_fp8(const uint16_t* x, uint8_t* codes, float* scales, 
   return e == cudaSuccess ? Q4T_OK : fail_cuda("row quantiser launch", e);
 }
 
+int32_t q4t_linear_check(const q4t_linear_args* l) {
+  if (!l) return fail(Q4T_ERR_INVALID, "null arguments");
+  LinearStrides s;
+  return l->M <= 0 ? Q4T_OK : check_linear(l, &s);
+}
+
 int32_t q4t_linear(const q4t_linear_args* l, void* stream) {
   if (!l) return fail(Q4T_ERR_INVALID, "null arguments");
   if (l->M <= 0) return Q4T_OK;
-  if (l->N <= 0 || l->K <= 0) return fail(Q4T_ERR_INVALID, "invalid GEMM dims");
-  if (!l->x || !l->w || !l->out) return fail(Q4T_ERR_INVALID, "null pointer");
-  if (l->activation < 0 || l->activation > Q4T_ACT_GELU) return fail(Q4T_ERR_INVALID, "unknown activation");
-  if (!l->fp8 && (l->x_scale || l->w_scale)) return fail(Q4T_ERR_INVALID, "scales belong to e4m3 operands");
-  const int64_t esz = l->fp8 ? 1 : 2;
-  // the stride of a single row is never used: any length of it will do
-  const int64_t one = (static_cast<int64_t>(l->K) + 15) & ~int64_t{15};
-  const int64_t ldx = l->M == 1 ? one : (l->ldx ? l->ldx : l->K), ldw = l->N == 1 ? one : (l->ldw ? l->ldw : l->K);
-  const int64_t ldo = l->ldo ? l->ldo : l->N, ldr = l->M == 1 ? ldo : (l->ldr ? l->ldr : l->N);
-  if (ldx < l->K || ldw < l->K || ldo < l->N || ldr < l->N) return fail(Q4T_ERR_INVALID, "a row stride is shorter than its row");
-  if (((reinterpret_cast<uintptr_t>(l->x) | reinterpret_cast<uintptr_t>(l->w)) & 15u) || (ldx * esz) % 16 || (ldw * esz) % 16)
-    return fail(Q4T_ERR_INVALID, "x and w must start at, and their rows be a multiple of, 16 bytes");
-  if (reinterpret_cast<uintptr_t>(l->out) % (l->out_f32 ? 4 : 2) || reinterpret_cast<uintptr_t>(l->residual) % 2 ||
-      reinterpret_cast<uintptr_t>(l->bias) % 2 || (reinterpret_cast<uintptr_t>(l->x_scale) | reinterpret_cast<uintptr_t>(l->w_scale)) % 4)
-    return fail(Q4T_ERR_INVALID, "out, residual, bias and scales must be aligned to their types");
-  if (l->residual && static_cast<const void*>(l->residual) == l->out && (l->out_f32 || ldr != ldo))
-    return fail(Q4T_ERR_INVALID, "in place, out and residual need the same type and row stride");
-  if (too_far(l->M, ldx, esz) || too_far(l->N, ldw, esz) || too_far(l->M, ldo, 4) || too_far(l->M, ldr, 2) || l->M > (1 << 30) || l->N > (1 << 30) || l->K > (1 << 29) || static_cast<int64_t>(l->N / 128 + 1) * (l->M / 16 + 1) > (1 << 30))
-    return fail(Q4T_ERR_INVALID, "dims too large");
-  // every output is finished by the thread that read its residual element: only there may the two be one
-  const bool in_place = static_cast<const void*>(l->residual) == l->out;
-  if (const char* on = covered(span_of(l->out, l->M, l->N, ldo, l->out_f32 ? 4 : 2),
-                               {{"x", span_of(l->x, l->M, l->K, ldx, esz)},
-                                {"w", span_of(l->w, l->N, l->K, ldw, esz)},
-                                {"x_scale", span_of(l->x_scale, int64_t{4} * l->M)},
-                                {"w_scale", span_of(l->w_scale, int64_t{4} * l->N)},
-                                {"bias", span_of(l->bias, int64_t{2} * l->N)},
-                                {"residual", span_of(in_place ? nullptr : l->residual, l->M, l->N, ldr, 2)}}))
-    return fail_overlap("out", on);
-  const DeviceState* ds;
-  int rc = device_state(&ds);
+  LinearStrides s;
+  int rc = check_linear(l, &s);
   if (rc != Q4T_OK) return rc;
+  const int64_t esz = l->fp8 ? 1 : 2, ldx = s.ldx, ldw = s.ldw, ldo = s.ldo, ldr = s.ldr;
+  const DeviceState* ds;
+  if ((rc = device_state(&ds)) != Q4T_OK) return rc;
   q4t::LinearArgs a{};
   a.M = l->M;
   a.N = l->N;
@@ -1877,47 +1934,19 @@ size_t q4t_verify_drafts_workspace_bytes(int32_t B, int32_t n, int32_t V) {
   return static_cast<size_t>(B) * (2 * n + 1) * static_cast<size_t>(q4t::verify_parts(V)) * sizeof(q4t::VerifyPart);
 }
 
+int32_t q4t_verify_drafts_check(const q4t_verify_args* v, const void* workspace, size_t workspace_bytes) {
+  if (!v) return fail(Q4T_ERR_INVALID, "null arguments");
+  return v->B <= 0 ? Q4T_OK : check_verify(v, workspace, workspace_bytes);
+}
+
 int32_t q4t_verify_drafts(const q4t_verify_args* v, void* workspace, size_t workspace_bytes, void* stream) {
   if (!v) return fail(Q4T_ERR_INVALID, "null arguments");
   if (v->B <= 0) return Q4T_OK;
-  if (v->n <= 0 || v->n > q4t::kVerifyMaxDrafts) return fail(Q4T_ERR_INVALID, "n out of range (1..64)");
-  if (v->V <= 0 || v->V > (1 << 30)) return fail(Q4T_ERR_INVALID, "V out of range (1..2^30)");
-  if (static_cast<int64_t>(v->B) * (2 * v->n + 1) > q4t::kVerifyMaxRows)
-    return fail(Q4T_ERR_INVALID, "too many rows: B * (2n + 1) is at most 65535");
-  if (!v->target_logits || !v->draft_ids || !v->uniforms || !v->tokens || !v->accepted)
-    return fail(Q4T_ERR_INVALID, "null pointer");
-  const int64_t tld = v->target_ld ? v->target_ld : v->V, dld = v->draft_ld ? v->draft_ld : v->V;
-  if (tld < v->V || dld < v->V) return fail(Q4T_ERR_INVALID, "a row stride is shorter than V");
-  if (too_far(q4t::kVerifyMaxRows, tld, 4) || too_far(q4t::kVerifyMaxRows, dld, 4)) return fail(Q4T_ERR_INVALID, "dims too large");
-  const uintptr_t esz = v->logits_f32 ? 4 : 2;
-  if ((reinterpret_cast<uintptr_t>(v->target_logits) | reinterpret_cast<uintptr_t>(v->draft_logits)) % esz)
-    return fail(Q4T_ERR_INVALID, "logits must be aligned to their type");
-  if ((reinterpret_cast<uintptr_t>(v->draft_ids) | reinterpret_cast<uintptr_t>(v->draft_len) | reinterpret_cast<uintptr_t>(v->temperature) |
-       reinterpret_cast<uintptr_t>(v->uniforms) | reinterpret_cast<uintptr_t>(v->tokens) | reinterpret_cast<uintptr_t>(v->accepted) |
-       reinterpret_cast<uintptr_t>(v->probs)) & 3u)
-    return fail(Q4T_ERR_INVALID, "ids, lengths, temperatures, uniforms and outputs must be 4-byte aligned");
-  const size_t need = q4t_verify_drafts_workspace_bytes(v->B, v->n, v->V);
-  if (!workspace || workspace_bytes < need) return fail(Q4T_ERR_WORKSPACE, "workspace too small");
-  if (reinterpret_cast<uintptr_t>(workspace) & 15u) return fail(Q4T_ERR_INVALID, "workspace must be 16-byte aligned");
-  const int64_t B = v->B, n = v->n;
-  const std::pair<const char*, Span> written[4] = {{"tokens", span_of(v->tokens, B * (n + 1) * 4)},
-                                                   {"accepted", span_of(v->accepted, B * 4)},
-                                                   {"probs", span_of(v->probs, B * (n + 1) * 4)},
-                                                   {"workspace", span_of(workspace, static_cast<int64_t>(need))}};
-  const std::pair<const char*, Span> read[6] = {{"target_logits", span_of(v->target_logits, B * (n + 1), v->V, tld, static_cast<int64_t>(esz))},
-                                                {"draft_logits", span_of(v->draft_logits, B * n, v->V, dld, static_cast<int64_t>(esz))},
-                                                {"draft_ids", span_of(v->draft_ids, B * n * 4)},
-                                                {"draft_len", span_of(v->draft_len, B * 4)},
-                                                {"temperature", span_of(v->temperature, B * 4)},
-                                                {"uniforms", span_of(v->uniforms, B * (n + 1) * 4)}};
-  for (int i = 0; i < 4; ++i) {
-    if (const char* on = covered(written[i].second, read)) return fail_overlap(written[i].first, on);
-    for (int j = 0; j < i; ++j)
-      if (overlap(written[i].second, written[j].second)) return fail_overlap(written[i].first, written[j].first);
-  }
-  const DeviceState* ds;
-  int rc = device_state(&ds);
+  int rc = check_verify(v, workspace, workspace_bytes);
   if (rc != Q4T_OK) return rc;
+  const int64_t tld = v->target_ld ? v->target_ld : v->V, dld = v->draft_ld ? v->draft_ld : v->V;
+  const DeviceState* ds;
+  if ((rc = device_state(&ds)) != Q4T_OK) return rc;
   const q4t::VerifyArgs a{v->target_logits, v->draft_logits, tld, dld, v->B, v->n, v->V, v->draft_ids, v->draft_len,
                           v->temperature, v->uniforms, v->tokens, v->accepted, v->probs,
                           static_cast<q4t::VerifyPart*>(workspace)};

@@ -6,6 +6,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <string>
 
 #include "q4t/status.h"
 #include "q4t_moe_b200.h"
@@ -50,6 +51,30 @@ inline VerifyHeadLayout LayoutOf(int B, int n, int hs, int vocab) {
   L.total = L.verify + up(q4t_verify_drafts_workspace_bytes(B, n, vocab));
   return L;
 }
+
+// What the step writes (workspace, outputs, with y also x) lies over nothing else of the step.
+inline Status Disjoint(const uint16_t* x, const uint16_t* y, const VerifyHeadWeights& w, const DraftBatch& b, const void* workspace,
+                       size_t workspace_bytes) {
+  struct Buffer {
+    const char* name;
+    const void* p;
+    size_t bytes;
+  };
+  const size_t rows = static_cast<size_t>(b.B) * (b.n + 1), drafts = static_cast<size_t>(b.B) * b.n, hs = w.hs, vocab = w.vocab;
+  const Buffer all[] = {{"workspace", workspace, workspace_bytes}, {"tokens", b.tokens, rows * 4}, {"accepted", b.accepted, b.B * size_t{4}},
+                        {"probs", b.probs, rows * 4}, {"x", x, rows * hs * 2}, {"y", y, rows * hs * 2}, {"norm", w.norm, hs * 2},
+                        {"head", w.head, vocab * hs}, {"head_scale", w.head_scale, vocab * 4}, {"draft_ids", b.draft_ids, drafts * 4},
+                        {"draft_len", b.draft_len, b.B * size_t{4}}, {"temperature", b.temperature, b.B * size_t{4}},
+                        {"uniforms", b.uniforms, rows * 4}, {"draft_logits", b.draft_logits, drafts * vocab * 2}};
+  const int count = sizeof(all) / sizeof(all[0]), written = y ? 5 : 4;
+  for (int i = 0; i < written; ++i)
+    for (int j = i + 1; j < count; ++j) {
+      const uintptr_t p = reinterpret_cast<uintptr_t>(all[i].p), q = reinterpret_cast<uintptr_t>(all[j].p);
+      if (p && q && p < q + all[j].bytes && q < p + all[i].bytes && !(all[i].p == x && all[j].p == y && x == y))
+        return Status::Fail(std::string("verify head: ") + all[j].name + " overlaps " + all[i].name);
+    }
+  return Status();
+}
 }  // namespace detail
 
 inline size_t VerifyHeadWorkspaceBytes(int B, int n, int hs, int vocab) {
@@ -57,7 +82,8 @@ inline size_t VerifyHeadWorkspaceBytes(int B, int n, int hs, int vocab) {
 }
 
 // x: residual stream bf16 [B*(n+1), hs], 16-byte aligned; y (may be null) is added to it first, in place.  Everything is
-// enqueued on `stream`.  logits_out (may be null) receives the address of the bf16 logits in the workspace.
+// enqueued on `stream`.  logits_out (may be null) receives the address of the bf16 logits in the workspace.  What is written (workspace,
+// 16-byte aligned, outputs, with y also x) may not lie over anything else.  A refused call has changed nothing.
 inline Status VerifyHead(uint16_t* x, const uint16_t* y, const VerifyHeadWeights& w, const DraftBatch& batch, void* workspace,
                          size_t workspace_bytes, cudaStream_t stream, const uint16_t** logits_out = nullptr) {
   const size_t need = VerifyHeadWorkspaceBytes(batch.B, batch.n, w.hs, w.vocab);
@@ -70,9 +96,6 @@ inline Status VerifyHead(uint16_t* x, const uint16_t* y, const VerifyHeadWeights
   float* scales = reinterpret_cast<float*>(base + L.scales);
   uint16_t* logits = reinterpret_cast<uint16_t*>(base + L.logits);
   const int rows = batch.B * (batch.n + 1);
-  if (q4t_residual_rmsnorm_fp8(x, y, y ? x : nullptr, w.norm, w.norm_offset, base + L.codes, scales, nullptr, rows, w.hs,
-                               w.eps, stream) != Q4T_OK)
-    return Status::Fail(q4t_last_error());
   q4t_linear_args l{};
   l.x = base + L.codes;
   l.w = w.head;
@@ -83,7 +106,6 @@ inline Status VerifyHead(uint16_t* x, const uint16_t* y, const VerifyHeadWeights
   l.x_scale = scales;
   l.w_scale = w.head_scale;
   l.out = logits;
-  if (q4t_linear(&l, stream) != Q4T_OK) return Status::Fail(q4t_last_error());
   q4t_verify_args v{};
   v.target_logits = logits;
   v.draft_logits = batch.draft_logits;
@@ -97,7 +119,16 @@ inline Status VerifyHead(uint16_t* x, const uint16_t* y, const VerifyHeadWeights
   v.tokens = batch.tokens;
   v.accepted = batch.accepted;
   v.probs = batch.probs;
-  if (q4t_verify_drafts(&v, base + L.verify, workspace_bytes - L.verify, stream) != Q4T_OK) return Status::Fail(q4t_last_error());
+  // everything that is refused is refused before x changes: the later calls' arguments, and buffers of one call over another's
+  const size_t verify_bytes = workspace_bytes - L.verify;
+  if (q4t_linear_check(&l) != Q4T_OK || q4t_verify_drafts_check(&v, base + L.verify, verify_bytes) != Q4T_OK)
+    return Status::Fail(q4t_last_error());
+  if (Status s = detail::Disjoint(x, y, w, batch, workspace, need); !s.ok()) return s;
+  if (q4t_residual_rmsnorm_fp8(x, y, y ? x : nullptr, w.norm, w.norm_offset, base + L.codes, scales, nullptr, rows, w.hs,
+                               w.eps, stream) != Q4T_OK)
+    return Status::Fail(q4t_last_error());
+  if (q4t_linear(&l, stream) != Q4T_OK) return Status::Fail(q4t_last_error());
+  if (q4t_verify_drafts(&v, base + L.verify, verify_bytes, stream) != Q4T_OK) return Status::Fail(q4t_last_error());
   if (logits_out) *logits_out = logits;
   return Status();
 }

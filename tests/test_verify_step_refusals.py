@@ -289,3 +289,24 @@ def test_draft_logits_in_the_logits_of_the_step_are_refused(q4t, step):
         with pytest.raises(q4t.Q4TError, match="head's own logits"):
             head(torch.zeros(6, 256, dtype=torch.bfloat16), IDS, U, draft_logits=bad)
     assert not ran
+
+
+def test_checks_alone(lib, q4t):
+    """The checks refuse what the calls refuse, without a GPU; what they accept they only look at."""
+    base = 1 << 20
+    good = q4t.LinearArgs(base, 2 * base, 4, 8, 64, 0, 0, 0, None, None, None, 0, 0, None, 0, 0, 3 * base)
+    assert lib.q4t_linear_check(C.byref(good)) == 0
+    refused(lib, lib.q4t_linear_check(None), "null")
+    good.out = base + 2
+    refused(lib, lib.q4t_linear_check(C.byref(good)), "out overlaps x")
+    good.M = 0
+    assert lib.q4t_linear_check(C.byref(good)) == 0
+    need = lib.q4t_verify_drafts_workspace_bytes(4, 3, 1000)
+    v = q4t.VerifyArgs(base, None, 0, 0, 0, 4, 3, 1000, 2 * base, None, None, 3 * base, 4 * base, 5 * base, None)
+    assert lib.q4t_verify_drafts_check(C.byref(v), 6 * base, need) == 0
+    assert lib.q4t_verify_drafts_check(C.byref(v), 6 * base, need - 1) == -2
+    refused(lib, lib.q4t_verify_drafts_check(None, 6 * base, need), "null")
+    v.accepted = 4 * base + 60
+    refused(lib, lib.q4t_verify_drafts_check(C.byref(v), 6 * base, need), "accepted overlaps tokens")
+    v.B = 0
+    assert lib.q4t_verify_drafts_check(C.byref(v), 6 * base, need) == 0
