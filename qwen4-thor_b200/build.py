@@ -2,7 +2,8 @@
 libq4t_moe_b200_check.so (device-side checkers used only by the GPU tests) for
 sm_100a with nvcc, and q4t_calls.so (the Python binding's compiled argument
 checks, host code on PyTorch's headers) with g++, in-tree, so that the shared
-objects travel with the source tree.
+objects travel with the source tree.  Without PyTorch the last one is left out:
+C and C++ programs do not need it.
 
     python qwen4-thor_b200/build.py [--force] [--verbose]
 """
@@ -32,10 +33,14 @@ def _newest_source() -> float:
 
 
 def _start_calls():
-    """The compile command of the Python binding's module, running."""
+    """The compile command of the Python binding's module, running; None where there is no PyTorch to compile it on."""
     import sysconfig
-    import torch
-    from torch.utils.cpp_extension import include_paths
+    try:
+        import torch
+        from torch.utils.cpp_extension import include_paths
+    except ImportError as e:
+        print(f"{os.path.basename(CALLS)} is left out: {e} (the Python binding's calls need it, C and C++ programs do not)", file=sys.stderr)
+        return None
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     includes = [*include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
