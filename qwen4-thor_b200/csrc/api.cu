@@ -44,6 +44,7 @@ using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, voi
 
 struct DeviceState {
   bool ready = false;
+  bool linear_ready = false, verify_ready = false;   // set-up that only q4t_linear and q4t_verify_drafts need
   int num_sms = 0;
   EncodeFn encode = nullptr;
   // The shared expert depends only on x, so q4t_moe_forward runs it on this
@@ -190,8 +191,9 @@ int check_verify(const q4t_verify_args* v, const void* workspace, size_t workspa
 }
 
 // Per-device one-time set-up: architecture check, driver entry point for the
-// tensor-map encoder, shared-memory attribute of the GEMM kernels.
-int device_state(const DeviceState** out) {
+// tensor-map encoder, shared-memory attribute of the GEMM kernels.  `more` sets up what one operator alone
+// needs, once per device (`done`): setting an attribute loads its kernel, which every program's first call would pay for.
+int device_state(const DeviceState** out, cudaError_t (*more)() = nullptr, bool DeviceState::*done = nullptr) {
   // every compute entry point passes here first: its first kernel follows the caller's
   // own stream work and is launched the ordinary way
   q4t::chain_break();
@@ -217,11 +219,13 @@ int device_state(const DeviceState** out) {
     if ((e = q4t::routing_set_attributes()) != cudaSuccess) return fail_cuda("cudaFuncSetAttribute", e);
     if ((e = q4t::small_batch_set_attributes()) != cudaSuccess) return fail_cuda("cudaFuncSetAttribute", e);
     if ((e = q4t::bf16_small_m_set_attributes()) != cudaSuccess) return fail_cuda("cudaFuncSetAttribute", e);
-    if ((e = q4t::linear_set_attributes()) != cudaSuccess) return fail_cuda("cudaFuncSetAttribute", e);
-    if ((e = q4t::verify_set_attributes()) != cudaSuccess) return fail_cuda("cudaFuncSetAttribute", e);
     s.encode = reinterpret_cast<EncodeFn>(fn);
     s.num_sms = prop.multiProcessorCount;
     s.ready = true;
+  }
+  if (more && !(s.*done)) {
+    if ((e = more()) != cudaSuccess) return fail_cuda("cudaFuncSetAttribute", e);
+    s.*done = true;
   }
   DeviceState& mine = t_lanes.dev[dev];
   if (!mine.ready) {
@@ -1890,7 +1894,7 @@ int32_t q4t_linear(const q4t_linear_args* l, void* stream) {
   if (rc != Q4T_OK) return rc;
   const int64_t esz = l->fp8 ? 1 : 2, ldx = s.ldx, ldw = s.ldw, ldo = s.ldo, ldr = s.ldr;
   const DeviceState* ds;
-  if ((rc = device_state(&ds)) != Q4T_OK) return rc;
+  if ((rc = device_state(&ds, q4t::linear_set_attributes, &DeviceState::linear_ready)) != Q4T_OK) return rc;
   q4t::LinearArgs a{};
   a.M = l->M;
   a.N = l->N;
@@ -1946,7 +1950,7 @@ int32_t q4t_verify_drafts(const q4t_verify_args* v, void* workspace, size_t work
   if (rc != Q4T_OK) return rc;
   const int64_t tld = v->target_ld ? v->target_ld : v->V, dld = v->draft_ld ? v->draft_ld : v->V;
   const DeviceState* ds;
-  if ((rc = device_state(&ds)) != Q4T_OK) return rc;
+  if ((rc = device_state(&ds, q4t::verify_set_attributes, &DeviceState::verify_ready)) != Q4T_OK) return rc;
   const q4t::VerifyArgs a{v->target_logits, v->draft_logits, tld, dld, v->B, v->n, v->V, v->draft_ids, v->draft_len,
                           v->temperature, v->uniforms, v->tokens, v->accepted, v->probs,
                           static_cast<q4t::VerifyPart*>(workspace)};
