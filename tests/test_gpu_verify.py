@@ -285,3 +285,45 @@ def test_shifted_drafts_of_long_rows_leave_no_difference(q4t, gpu_lib):
     assert torch.equal(s["draft"].float(), s["target"][:, :2].float() + 8)
     s["u"][:, 0] = 1.5
     compare(run(q4t, s), expect(s))
+
+
+def second_chunks(B, n, V, seed, draft, f32):
+    """Rows of which a warp of the first kernel takes two chunks (512 fp32 or 1024 bf16 tokens), with what one chunk of a pair may hold."""
+    L = 512 if f32 else 1024
+    s = make(B, n, V, seed, draft, f32, ragged=True, greedy=6)
+    parts = [s["target"]] + ([s["draft"]] if draft else [])
+    for t in parts:
+        t[0, :, 3 * L + 17] += 40.0                # maxima in the second chunk of a pair
+        t[6, :, L + 5] += 40.0
+        t[7, :, 5] += 30.0                          # a first chunk's maximum raised by the second's
+        t[7, :, L + 9] += 33.0
+        t[8, :, :L - 16] = float("-inf")            # the first, the second, both (and their neighbours)
+        t[9, :, L - 16:2 * L + 16] = float("-inf")
+        t[10, :, 2 * L - 16:4 * L + 16] = float("-inf")
+        t[11, :, L + 3] = float("nan")
+        t[12, :, 3 * L:4 * L] = float("nan")
+        t[13, :, :L] = float("nan")
+        t[1, :, 3 * L:3 * L + 40] = float("nan")    # greedy sequences
+        t[2, :, :2 * L] = float("-inf")
+        t[3, :, L + 200] = 60.0
+        t[3, :, 3 * L + 200] = 60.0
+        t[14] = torch.finfo(t.dtype).min
+        t[15, :, :] = float("-inf")
+        t[15, :, 2 * L + L // 2:2 * L + L // 2 + L] = 0.0
+        t[16, :, V - 1] += 50.0
+    s["target"][17, 0, L + 8] = float("inf")
+    s["lens"][:18] = n
+    return s
+
+
+@pytest.mark.parametrize("B,n,V,draft,f32", [(64, 3, 16391, False, True), (32, 7, 20011, True, False), (40, 5, 8200, True, True), (64, 7, 12000, False, False)])
+def test_second_chunks(q4t, gpu_lib, B, n, V, draft, f32):
+    rows_ = B * (n + 1 + (n if draft else 0))
+    per = 512 if f32 else 1024
+    assert rows_ * ((V + 8 + per - 1) // per) // 2 >= 148 * 20     # the first kernel's rule for two chunks a warp
+    s = second_chunks(B, n, V, V, draft, f32)
+    want = expect(s)
+    compare(run(q4t, s), want)
+    compare(run(q4t, s, (V + 8) // 8 * 8 + 3), want)
+    s["u"][:, 0] = 1.5                                             # every first draft refused
+    compare(run(q4t, s), expect(s))
