@@ -193,3 +193,37 @@ def test_codes_of_a_norm_are_the_division(q4t, gpu_lib, T, hs):
         want, swant = division(sign * (w.float() + 0.0))   # the offset of zero takes the weight's -0 away
         assert torch.equal(scales, swant)
         assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8))
+
+
+def behind(rows, width, dtype, fill):
+    return torch.full((rows + 3, width), fill, dtype=dtype, device="cuda")
+
+
+@pytest.mark.parametrize("T,hs", [(1025, 8), (1033, 256), (1030, 264), (1029, 512), (1025, 520), (1030, 2560), (1027, 8192), (3, 8200), (1026, 8200),
+                                  (2, 16384), (1025, 16392), (16385, 72)])
+@pytest.mark.parametrize("with_y,with_w,offset,with_h", [(True, True, 1.0, True), (False, False, 0.0, False)])
+def test_norm_of_many_and_of_long_rows(q4t, gpu_lib, T, hs, with_y, with_w, offset, with_h):
+    """The forms that row counts above 1024 and row lengths choose; rows behind the last stay as they were."""
+    x, y, w = inputs(T, hs, T + hs, spread=3.0)
+    y, w = y if with_y else None, w if with_w else None
+    codes, scales = behind(T, hs, torch.uint8, 0x55), behind(T, 1, torch.float32, -1.0)
+    x_out = behind(T, hs, torch.bfloat16, 5.0) if with_y else None
+    h = behind(T, hs, torch.bfloat16, 6.0) if with_h else None
+    q4t.residual_rmsnorm_fp8(x, y, w, codes[:T].view(torch.float8_e4m3fn), scales[:T, 0], x_out=None if x_out is None else x_out[:T],
+                             h=None if h is None else h[:T], eps=1e-6, weight_offset=offset)
+    r, v = formula(x, y, w, offset, 1e-6)
+    if with_y:
+        assert torch.equal(x_out[:T], r) and (x_out[T:] == 5).all()
+    if with_h:
+        assert ((h[:T].double() - v).abs() <= v.abs() * (2.0 ** -8 + 2 * REL)).all() and (h[T:] == 6).all()
+    check_rows(codes[:T].view(torch.float8_e4m3fn), scales[:T, 0], v)
+    assert (codes[T:] == 0x55).all() and (scales[T:] == -1).all()
+
+
+@pytest.mark.parametrize("rows,K", [(1027, 72), (1025, 256), (1031, 504), (1029, 1016), (1026, 1032), (1026, 2048), (1025, 16384), (1025, 16392), (9, 8200)])
+def test_quantiser_of_many_and_of_long_rows(q4t, gpu_lib, rows, K):
+    x, _, _ = inputs(rows, K, rows + K, spread=0.02)
+    codes, scales = behind(rows, K, torch.uint8, 0x55), behind(rows, 1, torch.float32, -1.0)
+    q4t.quantize_rows_fp8(x, codes[:rows].view(torch.float8_e4m3fn), scales[:rows, 0])
+    check_rows(codes[:rows].view(torch.float8_e4m3fn), scales[:rows, 0], x.double())
+    assert (codes[rows:] == 0x55).all() and (scales[rows:] == -1).all()
