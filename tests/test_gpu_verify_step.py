@@ -247,3 +247,24 @@ def test_overlapping_draft_rows_are_refused_before_x_changes(q4t, gpu_lib):
         with pytest.raises(q4t.Q4TError):
             head(x, ids, u, y=x.clone(), draft_logits=bad)
     assert torch.equal(x, before)
+
+
+@pytest.mark.parametrize("B,n,hs,V", [(1, 1, 256, 517), (4, 3, 512, 3001), (8, 3, 2048, 8192), (3, 7, 1040, 1000)])
+def test_logits_of_the_e4m3_head(q4t, gpu_lib, B, n, hs, V):
+    """The head's logits are the product of what its norm and its weight's layout left, in 64 bits: at most hs / 32 + 32 additions
+    of an fp32 ulp of S each, four fp32 roundings, and one bf16 rounding.  Against the product of the unrounded operands the whole error is the two
+    e4m3 roundings': each uniform within 2^-4 of a value at most, so 2^-4 / sqrt(3) in the root mean square, in quadrature, relative to the
+    root of the summed squares; a quarter more covers the spread over a finite number of logits, the codes below 2^-6 and the bf16 rounding."""
+    T = B * (n + 1)
+    nw, w = head_weights(V, hs, V)
+    head = q4t.VerifyHead(nw, w, B, n)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = (2 * torch.randn(T, hs, generator=g, device="cuda")).bfloat16()
+    head(x, torch.zeros(B, n, dtype=torch.int32, device="cuda"), torch.rand(B, n + 1, generator=g, device="cuda"))
+    a, b = head.codes.float().double() * head.scales.double()[:, None], head.head.float().double() * head.head_scale.double()[:, None]
+    want, S = a @ b.t(), a.abs() @ b.abs().t()
+    tol = ((hs / 32 + 32) * 2.0 ** -23 + 4 * 2.0 ** -24) * S
+    assert ((head.logits.double() - want).abs() <= tol + 2.0 ** -8 * (want.abs() + tol)).all()
+    v = x.double() / (x.double().square().mean(1, keepdim=True) + 1e-6).sqrt() * nw.double()
+    S2 = (v.square() @ w.double().square().t()).sqrt()
+    assert float((head.logits.double() - v @ w.double().t()).norm() / S2.norm()) <= 1.25 * 2.0 ** 0.5 * 2.0 ** -4 / 3.0 ** 0.5
