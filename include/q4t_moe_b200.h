@@ -636,7 +636,10 @@ int32_t q4t_linear_status(void);
  * no probability, +inf counts as the largest finite value.  A draft id outside [0, V)
  * does not stand; neither does a draft whose target row has no probability at all, and the
  * token drawn there is -1.  draft_len outside [0, n] is clamped.  Rows behind a sequence's
- * drafts are not read.  The weights, sums and differences of the drawn row are 64-bit.
+ * drafts are not read.  The weights, sums and differences of the drawn row are 64-bit (which of its tokens
+ * have p > q is decided at 1e-7 as long as that shifts no border of the draw by more than 2^-16 of what is left
+ * to draw from, exactly otherwise); acceptances and the probabilities of drafts that stand come from
+ * fp32 exponentials with 64-bit sums (2^-20 of the value).
  * No output may overlap another buffer (refused).  Deterministic; no host synchronisation.
  * Calls that share a workspace must not run at the same time.                     */
 typedef struct q4t_verify_args {

@@ -23,7 +23,10 @@
 // One pass over the drawn row is enough although p - q needs both sums first: a weight is counted into
 // P = sum of e^p and Q = sum of e^q over the tokens with p > q by the first kernel's sums (good to 1e-7), while the exact
 // sums A and B of all e^p and e^q are formed beside them; then sum(r) = P / A - Q / B.  A token on the wrong side of the
-// comparison has |p - q| <= 1e-7 p, and the tokens that close to the border hold about 1e-7 of the mass: 1e-14.
+// comparison has |p - q| <= d p, d the relative error of the first kernel's ratio of sums (1e-7), so no border of the draw is off by
+// more than d, and where p / q spreads by much more than d by about d^2.  d is known once the exact sums are; where it is more
+// than 2^-16 of what there is to draw from (distributions that agree to a percent, whose drafts are as rarely refused), a second pass
+// compares with the exact ratio.  (Before that, rows that agreed to 1e-7 drew one token in ten wrongly; 0.2 to 0.5 us a call.)
 #include <math_constants.h>
 
 #include "kernels.h"
@@ -39,6 +42,8 @@ constexpr int kDrawCtas = 8;   // most CTAs of a sequence
 constexpr float kF32Max = 3.402823466e38f;
 // A difference p - q that adds up to this (2^-40) or less is what 64-bit sums of equal distributions leave.
 constexpr double kNothing = 9.094947017729282e-13;
+// How far tokens on the wrong side of the comparison p > q may shift a border of the draw, relative to what is drawn from: 2^-16.
+constexpr double kShift = 1.52587890625e-5;
 
 // NaN -> -inf, +inf -> the largest finite value.
 __device__ __forceinline__ float clean_logit(float l) { return fminf(fmaxf(l, -CUDART_INF_F), kF32Max); }
@@ -340,6 +345,11 @@ __device__ __forceinline__ double exp2_low(double z, const double* table) { retu
 // the row's maximum, or 0 (see WeightTable).  Weights and sums of weights up to kTiny of the row's sum count as none (2^30
 // of the least are below it).
 constexpr double kTiny = 1.0e-265;   // about 2^-880
+__device__ __forceinline__ double row_weight(float l, float ref, double c, const double* table) {
+  const float v = clean_logit(l);
+  const double z = (static_cast<double>(v) - static_cast<double>(ref)) * c;
+  return v > -CUDART_INF_F && z > -1000.0 ? exp2_table(z, table) : 0.0;
+}
 struct RowWeights {
   double c, mc, cs;       // mc = ref c; cs = c * 2^896: a float's bits moved into a double's places are its value times 2^-896
   float m, ref, least;
@@ -357,11 +367,7 @@ struct RowWeights {
     least2 = f32x2_to_bf16x2(least, least);
   }
   // any row, one logit at a time
-  __device__ __forceinline__ double operator()(float l, const double* table) const {
-    const float v = clean_logit(l);
-    const double z = (static_cast<double>(v) - static_cast<double>(ref)) * c;
-    return v > -CUDART_INF_F && z > -1000.0 ? exp2_table(z, table) : 0.0;
-  }
+  __device__ __forceinline__ double operator()(float l, const double* table) const { return row_weight(l, ref, c, table); }
   // the logits of one word of a regular row: E / 4 of them
   template <bool F32>
   __device__ __forceinline__ void word(uint32_t w, const double* table, double* e) const {
@@ -437,9 +443,9 @@ struct DrawShared {
   uint8_t ok[kVerifyMaxDrafts];
   double table[16];
   double warp_sums[4][kDrawMaxWarps];                        // A, B, P, Q of each warp
-  double all[kDrawCtas][4];                                  // and of each CTA of the cluster
+  double all[2][kDrawCtas][4];                               // and of each CTA of the cluster, in either pass
   double lower, goal, sum, scale_q;                          // found by the first warp: see there
-  int share, plain;
+  int share, plain, again;
   int token;
   double prob;
 };
@@ -453,6 +459,26 @@ __device__ __forceinline__ double sum8(double v) {
 #pragma unroll
   for (int off = 1; off < 8; off <<= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
   return v;
+}
+
+// The four sums of a warp's tokens [t0, t1), token by token, with the exact scale of the draft row's weights.
+struct Sums {
+  double a, b, p, q;
+};
+template <bool F32>
+__device__ __noinline__ Sums exact_sums(Row<F32> rp, Row<F32> rq, int t0, int t1, double c, float ref_p, float ref_q, double scale_q,
+                                        const double* table) {
+  Sums s{0.0, 0.0, 0.0, 0.0};
+  for (int t = t0 + (threadIdx.x & 31); t < t1; t += 32) {
+    const double ep = row_weight(rp.one(t), ref_p, c, table), eq = row_weight(rq.one(t), ref_q, c, table);
+    s.a += ep;
+    s.b += eq;
+    if (ep > __dmul_rn(eq, scale_q)) {
+      s.p += ep;
+      s.q += eq;
+    }
+  }
+  return s;
 }
 
 // A cluster of gridDim.x CTAs per sequence: join the parts (1.3 us), accept, one pass over the drawn row, exchange the sums
@@ -585,8 +611,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_draw_kernel(co
     const int without = refused && !has_q ? a.draft_ids[static_cast<size_t>(b) * a.n + at] : -1;
     const float mq = minus_q ? sh.q[at].m : st.m;
     const bool looked = TABLE && WeightTable::built(c) && WeightTable::usable(st.m, c) && WeightTable::usable(mq, c);
-    const RowWeights wp(st.m, looked ? 0.0f : st.m, c, F32), wq(mq, looked ? 0.0f : mq, c, F32);
-    // p > q by the first kernel's sums: e^p * ratio > e^q
+    const RowWeights wp(st.m, looked ? 0.0f : st.m, c, F32), wq(mq, looked ? 0.0f : mq, c, F32);    // p > q by the first kernel's sums: e^p * ratio > e^q
     double ratio = minus_q ? sh.ratio[at] : 0.0;
     if (looked) ratio *= exp2_table((static_cast<double>(mq) - static_cast<double>(st.m)) * c, sh.table);
 
@@ -671,23 +696,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_draw_kernel(co
       };
       pass([&](uint32_t w, double* e) { careful(wp, w, e); }, [&](uint32_t w, double* e) { careful(wq, w, e); });
     }
-    sa = warp_sum(sa);
-    sb = warp_sum(sb);
-    sp = warp_sum(sp);
-    sq = warp_sum(sq);
-    if (lane == 0) {
-      sh.warp_sums[0][warp] = sa;
-      sh.warp_sums[1][warp] = sb;
-      sh.warp_sums[2][warp] = sp;
-      sh.warp_sums[3][warp] = sq;
-    }
-    __syncthreads();
-    if (warp < 4) {   // a sum each, to every CTA
-      const double t = warp_sum(lane < kDrawWarps ? sh.warp_sums[warp][lane] : 0.0);
-      if (lane < ctas) st_cluster_f64(cluster_map(smem_u32(&sh.all[cta][warp]), static_cast<uint32_t>(lane)), t);
-    }
-    __syncwarp();
-    cluster_sync();
     // The share (one a lane) that `goal` falls into, with what lies before it; rounding may leave the goal behind the last
     // share that holds anything.
     auto find = [&](double w, double upto, double goal, double none, double& lower) {
@@ -696,34 +704,63 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_draw_kernel(co
       lower = __shfl_sync(0xffffffffu, upto - w, k);
       return k;
     };
-    if (warp == 0) {   // the first warp of every CTA adds the CTAs' shares in the same order, a lane per share
-      const int c8 = lane & (kDrawCtas - 1);
-      const bool have_cta = c8 < ctas;
-      const double ka = have_cta ? sh.all[c8][0] : 0.0, kb = have_cta ? sh.all[c8][1] : 0.0;
-      const double kp = have_cta ? sh.all[c8][2] : 0.0, kq = have_cta ? sh.all[c8][3] : 0.0;
-      const double A = sum8(ka), B = sum8(kb), P = sum8(kp), Q = sum8(kq);
-      // everything in the measure of the target's weights, whose sum is A
-      const double scale_q = minus_q ? A / B : 0.0, none = kTiny * A;
-      const bool plain = !(P - Q * scale_q > kNothing * A);   // the difference leaves nothing: the target's own distribution
-      auto mass = [&](double wa, double wp_, double wq_) { return plain ? wa : fmax(wp_ - wq_ * scale_q, 0.0); };
-      const double wk = lane < ctas ? mass(ka, kp, kq) : 0.0, upto = warp_scan(wk);
-      const double goal = static_cast<double>(u_draw) * __shfl_sync(0xffffffffu, upto, 31);
-      double lower;
-      int share = -1;
-      if (find(wk, upto, goal, none, lower) == cta) {
-        const double ww = lane < kDrawWarps ? mass(sh.warp_sums[0][lane], sh.warp_sums[2][lane], sh.warp_sums[3][lane]) : 0.0;
-        share = find(ww, lower + warp_scan(ww), goal, none, lower);
-      }
+    // one turn, and in rare cases a second with the exact sums' ratio: see kShift
+#pragma unroll 1
+    for (int turn = 0;; ++turn) {
+      sa = warp_sum(sa);
+      sb = warp_sum(sb);
+      sp = warp_sum(sp);
+      sq = warp_sum(sq);
       if (lane == 0) {
-        sh.share = share;
-        sh.plain = plain;
-        sh.lower = lower;
-        sh.goal = goal;
-        sh.sum = A;
-        sh.scale_q = scale_q;
+        sh.warp_sums[0][warp] = sa;
+        sh.warp_sums[1][warp] = sb;
+        sh.warp_sums[2][warp] = sp;
+        sh.warp_sums[3][warp] = sq;
       }
+      __syncthreads();
+      if (warp < 4) {   // a sum each, to every CTA
+        const double t = warp_sum(lane < kDrawWarps ? sh.warp_sums[warp][lane] : 0.0);
+        if (lane < ctas) st_cluster_f64(cluster_map(smem_u32(&sh.all[turn][cta][warp]), static_cast<uint32_t>(lane)), t);
+      }
+      __syncwarp();
+      cluster_sync();
+      if (warp == 0) {   // the first warp of every CTA adds the CTAs' shares in the same order, a lane per share
+        const int c8 = lane & (kDrawCtas - 1);
+        const bool have_cta = c8 < ctas;
+        const double ka = have_cta ? sh.all[turn][c8][0] : 0.0, kb = have_cta ? sh.all[turn][c8][1] : 0.0;
+        const double kp = have_cta ? sh.all[turn][c8][2] : 0.0, kq = have_cta ? sh.all[turn][c8][3] : 0.0;
+        const double A = sum8(ka), B = sum8(kb), P = sum8(kp), Q = sum8(kq);
+        // everything in the measure of the target's weights, whose sum is A
+        const double scale_q = minus_q ? A / B : 0.0, none = kTiny * A;
+        const bool plain = !(P - Q * scale_q > kNothing * A);   // the difference leaves nothing: the target's own distribution
+        auto mass = [&](double wa, double wp_, double wq_) { return plain ? wa : fmax(wp_ - wq_ * scale_q, 0.0); };
+        const double wk = lane < ctas ? mass(ka, kp, kq) : 0.0, upto = warp_scan(wk);
+        const double goal = static_cast<double>(u_draw) * __shfl_sync(0xffffffffu, upto, 31);
+        const bool again = turn == 0 && minus_q && fabs(ratio * scale_q - 1.0) * A > kShift * (P - Q * scale_q);
+        double lower;
+        int share = -1;
+        if (find(wk, upto, goal, none, lower) == cta) {
+          const double ww = lane < kDrawWarps ? mass(sh.warp_sums[0][lane], sh.warp_sums[2][lane], sh.warp_sums[3][lane]) : 0.0;
+          share = find(ww, lower + warp_scan(ww), goal, none, lower);
+        }
+        if (lane == 0) {
+          sh.share = share;
+          sh.plain = plain;
+          sh.lower = lower;
+          sh.goal = goal;
+          sh.sum = A;
+          sh.scale_q = scale_q;
+          sh.again = again;
+        }
+      }
+      __syncthreads();
+      if (!sh.again) break;
+      const Sums sums = exact_sums<F32>(rp, rq, max(rp.first(first_piece), 0), min(rp.first(end_piece), a.V), c, wp.ref, wq.ref, sh.scale_q, sh.table);
+      sa = sums.a;
+      sb = sums.b;
+      sp = sums.p;
+      sq = sums.q;
     }
-    __syncthreads();
     const int share = sh.share;
     mine = share >= 0;
     if (mine) {

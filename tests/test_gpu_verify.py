@@ -327,3 +327,38 @@ def test_second_chunks(q4t, gpu_lib, B, n, V, draft, f32):
     compare(run(q4t, s, (V + 8) // 8 * 8 + 3), want)
     s["u"][:, 0] = 1.5                                             # every first draft refused
     compare(run(q4t, s), expect(s))
+
+
+def nearly_equal(B, V, seed, f32):
+    """Target and draft rows that agree to 1e-7, but for one unlikely token that the drafter favours and drafts.  fp32: noise of 2e-7 on every
+    logit; bf16: one token in eight, of a total probability of 4e-8, has another logit."""
+    g = torch.Generator().manual_seed(seed)
+    dt = torch.float32 if f32 else torch.bfloat16
+    t = (2.0 * torch.randn(B, 2, V, generator=g)).to(dt).float()
+    x = torch.randint(0, V, (B, 1), generator=g)
+    rare = torch.full((B, V), False)
+    for b in range(B):
+        rare[b, torch.randperm(V, generator=g)[:V // 8]] = True
+    if f32:
+        d = t[:, 0] + 2e-7 * torch.randn(B, V, generator=g)
+    else:
+        t[:, 0] = torch.where(rare, torch.full((B, V), -13.0), t[:, 0])
+        d = t[:, 0] + torch.where(rare, torch.randint(-1, 2, (B, V), generator=g).float(), torch.zeros(B, V))
+    t[:, 0].scatter_(1, x, -16.0)
+    d.scatter_(1, x, -14.0)
+    return {"target": t.to(dt), "draft": d[:, None].to(dt), "T": None, "u": torch.cat([torch.full((B, 1), 0.9), torch.rand(B, 1, generator=g)], 1),
+            "lens": None, "ids": x.int()}
+
+
+@pytest.mark.parametrize("B,V,seed,f32", [(24, 1001, 0, True), (24, 1001, 3, True), (12, 16000, 3, True), (12, 16000, 4, True), (2, 70001, 0, True),
+                                              (2, 70001, 3, True), (24, 5001, 3, False), (12, 16000, 2, False), (12, 16000, 20, False), (2, 70001, 1, False)])
+def test_draws_from_what_nearly_equal_distributions_leave(q4t, gpu_lib, B, V, seed, f32):
+    """The weights are good to 1.5e-13 each, so a border of the draw to 3e-13 of the whole and, relative to the little that is left of it, to 3e-13 / left."""
+    s = nearly_equal(B, V, seed, f32)
+    p, q = (torch.softmax(s[k][:, 0].double(), 1) for k in ("target", "draft"))
+    left = float((p - q).clamp_min(0).sum(1).min())
+    assert 1e-8 < left < 1e-6
+    tokens, accepted, probs, accept_margin, draw_margin = verify(
+        s["target"].float().numpy(), s["ids"].numpy(), s["u"].numpy(), s["draft"].float().numpy())
+    assert accept_margin > 2.0 ** -18 and draw_margin > 3e-13 / left and (accepted == 0).all()
+    compare(run(q4t, s), (tokens, accepted, probs))
