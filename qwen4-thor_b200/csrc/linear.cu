@@ -11,9 +11,9 @@
 // Rows and k past the ends of the operands are zeros from TMA; nothing is stored for them.
 //
 // On a B200 (copy 6.47 TB/s, cuBLAS bf16 1670 TFLOP/s in a burst and 1400 under the power cap): 16384 x 2048 x 2048 bf16 100 us
-// (1370 TFLOP/s; 111 with a residual; cuBLAS without one 100), 122 under the power cap (cuBLAS 115 to 118); 8192^3 bf16 1254
-// TFLOP/s under the cap (cuBLAS 1391); 8001 x 5120 x 2560 e4m3 88 us (2390 TFLOP/s; 96 with bias and GELU); 128 x 131072 x 2048 e4m3
-// 55 us (5.5 TB/s); one token against 2048 x 2048 3.3 us (linear_row_kernel).
+// (1370 TFLOP/s; 105 with a residual; cuBLAS without one 100), 122 under the power cap (cuBLAS 115 to 118); 8192^3 bf16 1254
+// TFLOP/s under the cap (cuBLAS 1391); 8001 x 5120 x 2560 e4m3 89 us (2360 TFLOP/s; 98 with bias and GELU); 128 x 131072 x 2048 e4m3
+// 56 us (5.4 TB/s), 66 repeated under the power cap; one token against 2048 x 2048 3.3 us (linear_row_kernel).
 #include <cuda_fp16.h>
 
 #include "kernels.h"

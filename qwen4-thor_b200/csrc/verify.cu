@@ -17,8 +17,8 @@
 // token a uniform falls on hangs on a sum of up to V weights next to a border, and with V borders fp32 sums would
 // miss one in a hundred draws, so the drawn row's weights, sums and differences are 64-bit throughout.
 //
-// On a B200, 32 sequences of 3 drafts over 131072 tokens, bf16 with draft logits (58.7 MB, 9.1 us at the copy rate): 34 us, 16 of
-// them the first kernel; one sequence over 32003 tokens, fp32: 9.9 us, nearly all of it latency.
+// On a B200, 32 sequences of 3 drafts over 131072 tokens, bf16 with draft logits (58.7 MB, 9.1 us at the copy rate): 35.5 us, 16 of
+// them the first kernel; one sequence over 32003 tokens, fp32: 10.2 us, nearly all of it latency.
 //
 // One pass over the drawn row is enough although p - q needs both sums first: a weight is counted into
 // P = sum of e^p and Q = sum of e^q over the tokens with p > q by the first kernel's sums (good to 1e-7), while the exact
